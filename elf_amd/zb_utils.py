@@ -204,15 +204,19 @@ LinearDW.register_dx_function(LinearDX)
 # ------------------------------------------------------------------------------------------------ 8 bits
 class _Kept8:
 	"""What a layer in 8 bits keeps of a micro-batch: its input or its output gradient along the tokens (``kernels.Fp8Rows`` of the
-	transpose, half of the bf16 bytes), and of an output gradient its sum over the tokens where there is a bias."""
+	transpose, half of the bf16 bytes), and of an output gradient its sum over the tokens where there is a bias.  ``use``: the forward call that an
+	output gradient belongs to; ``more``: what came before it of the same call (a stage goes back from its outputs one after the other)."""
 
-	__slots__ = ("rows", "bias")
+	__slots__ = ("rows", "bias", "use", "more")
 
-	def __init__(self, rows, bias=None):
-		self.rows, self.bias = rows, bias
+	def __init__(self, rows, bias=None, use=None, more=None):
+		self.rows, self.bias, self.use, self.more = rows, bias, use, more
 
 	def to(self, device, non_blocking=False):
-		return _Kept8(self.rows.to(device, non_blocking=non_blocking), None if self.bias is None else self.bias.to(device, non_blocking=non_blocking))
+		def there(part):
+			return None if part is None else part.to(device, non_blocking=non_blocking)
+
+		return _Kept8(there(self.rows), there(self.bias), self.use, there(self.more))
 
 
 def _forward8(x8, linear):
@@ -222,13 +226,13 @@ def _forward8(x8, linear):
 	return kernels.gemm_fp8(x8, w8, epilogue=kernels.EPI_BF16_RESID, residual=linear.bias.detach(), residual_ld=0)
 
 
-def _backward8(go, linear):
-	"""The input gradient; the output gradient is kept for W."""
+def _backward8(go, linear, use):
+	"""The input gradient of the forward call ``use``; the output gradient is kept for W."""
 	dy8, dy8t = kernels.quant_fp8(go, dtype=linear.grad_dtype, transposed=True)
 	bias = None
 	if linear.bias is not None:
 		bias = kernels.colsum_(go, torch.zeros(go.shape[1], dtype=torch.float32, device=go.device))
-	linear._store_grad_output(_Kept8(dy8t, bias))
+	linear._store_grad_output(_Kept8(dy8t, bias, use))
 	_, w8t = kernels.quant_fp8_weight(linear.weight.detach(), rows=False, transposed=True)
 	return kernels.gemm_fp8(dy8, w8t)
 
@@ -242,14 +246,14 @@ class Linear8DX(torch.autograd.Function):
 	def forward(ctx, input, weight, bias, linear):
 		x8, x8t = kernels.quant_fp8(_as_rows(input.detach()), transposed=True)
 		linear._store_input8(x8t)
-		ctx.linear, ctx.in_shape = linear, input.shape
+		ctx.linear, ctx.in_shape, ctx.use = linear, input.shape, object()
 		ctx.save_for_backward(x8t.memory)  # read again in B, so that torch.utils.checkpoint runs the forward again
 		return _forward8(x8, linear).view(*input.shape[:-1], weight.shape[0])
 
 	@staticmethod
 	def backward(ctx, grad_output):
 		ctx.saved_tensors  # noqa: B018
-		return _backward8(_as_rows(grad_output), ctx.linear).view(ctx.in_shape), None, None, None
+		return _backward8(_as_rows(grad_output), ctx.linear, ctx.use).view(ctx.in_shape), None, None, None
 
 
 class Linear8DW(LayerDW, Linear8):
@@ -272,8 +276,10 @@ class Linear8DW(LayerDW, Linear8):
 		self.__dict__["last_input"] = _Kept8(rows)
 
 	def _store_grad_output(self, kept):
-		if getattr(self, "last_grad_output", None) is not None:
+		last = getattr(self, "last_grad_output", None)
+		if last is not None and last.use is not kept.use:
 			raise _lib.ElfStageError(f"{type(self).__name__}: the layer was used several times in one forward (sums of output gradients in 8 bits would need bf16 again)")
+		kept.more = last
 		self.__dict__["last_grad_output"] = kept
 
 	_main_grad = LinearDW._main_grad
@@ -285,9 +291,11 @@ class Linear8DW(LayerDW, Linear8):
 	def backward(self, mb_id):
 		"""W: main_grad += dY^T X (fp32) from the two 8-bit matrices, bias main_grad += the sum that B left; drops the stash."""
 		kept, x = self.ctx["grad_output"][mb_id], self.ctx["input"][mb_id]
-		kernels.gemm_fp8(kept.rows, x.rows, out=self._main_grad(self.weight), epilogue=kernels.EPI_F32_ACC)
-		if self.bias is not None:
-			self._main_grad(self.bias).add_(kept.bias)
+		while kept is not None:
+			kernels.gemm_fp8(kept.rows, x.rows, out=self._main_grad(self.weight), epilogue=kernels.EPI_F32_ACC)
+			if self.bias is not None:
+				self._main_grad(self.bias).add_(kept.bias)
+			kept = kept.more
 		self.ctx["grad_output"][mb_id] = None
 		self.ctx["input"][mb_id] = None
 
@@ -301,7 +309,7 @@ class NormLinear8DX(torch.autograd.Function):
 		rows = None if residual is None else _as_rows(residual.detach())
 		h, n8, stats = kernels.rms_norm_fp8(_as_rows(x.detach()), gamma.detach(), residual=rows, eps=linear.eps)
 		linear._store_input8(kernels.transpose_fp8(n8))
-		ctx.linear, ctx.in_shape, ctx.added = linear, x.shape, residual is not None
+		ctx.linear, ctx.in_shape, ctx.use, ctx.added = linear, x.shape, object(), residual is not None
 		ctx.set_materialize_grads(False)
 		y = _forward8(n8, linear).view(*x.shape[:-1], weight.shape[0])
 		ctx.save_for_backward(h, stats, gamma)
@@ -314,7 +322,7 @@ class NormLinear8DX(torch.autograd.Function):
 		dx, dgamma = dh, None
 		if dy is not None:
 			acc = torch.zeros(gamma.shape, dtype=torch.float32, device=gamma.device)
-			dn = _backward8(_as_rows(dy), ctx.linear)
+			dn = _backward8(_as_rows(dy), ctx.linear, ctx.use)
 			dx = kernels.norm_bwd(kernels.NORM_RMS, dn, h, gamma.detach(), stats, acc, dres=None if dh is None else _as_rows(dh)).view(ctx.in_shape)
 			dgamma = acc.to(gamma.dtype)
 		return dx, dx if ctx.added else None, dgamma, None, None, None
