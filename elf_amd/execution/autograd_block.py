@@ -17,7 +17,7 @@ from torch.utils.checkpoint import checkpoint
 
 from .. import _lib
 from ..scheduling import OpOptions
-from ..zb_utils import LayerDW, LinearDW, replace_layer_with_layer_dw
+from ..zb_utils import LayerDW, LinearDW, NormLinear8DW, replace_layer_with_layer_dw
 from .block import StageBlockBase
 
 logger = logging.getLogger("block")
@@ -32,6 +32,10 @@ class AutogradStageBlock(StageBlockBase):
 		_lib.load()
 		self._init_common(model, id_, placement, signature, pp_group, dp_group, recv_pgs, send_pgs)
 		replace_layer_with_layer_dw(self.model)
+		norms = [m for m in self.model.modules() if isinstance(m, NormLinear8DW)]
+		elsewhere = {id(p) for m in self.model.modules() for p in m.parameters(recurse=False) if m not in norms}
+		for m in norms:
+			m.gain_in_main = id(m.gamma) not in elsewhere
 		logger.info(f"{self}: generic stage ({type(model).__name__}): linear layers on the HIP GEMM, the rest through PyTorch autograd")
 
 	def _layers_dw(self):

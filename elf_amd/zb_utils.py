@@ -204,19 +204,20 @@ LinearDW.register_dx_function(LinearDX)
 # ------------------------------------------------------------------------------------------------ 8 bits
 class _Kept8:
 	"""What a layer in 8 bits keeps of a micro-batch: its input or its output gradient along the tokens (``kernels.Fp8Rows`` of the
-	transpose, half of the bf16 bytes), and of an output gradient its sum over the tokens where there is a bias.  ``use``: the forward call that an
-	output gradient belongs to; ``more``: what came before it of the same call (a stage goes back from its outputs one after the other)."""
+	transpose, half of the bf16 bytes), and of an output gradient its sum over the tokens where there is a bias and the gradient of the gain where
+	there is a norm, both in fp32.  ``use``: the forward call that an output gradient belongs to; ``more``: what came before it of the same call (a
+	stage goes back from its outputs one after the other)."""
 
-	__slots__ = ("rows", "bias", "use", "more")
+	__slots__ = ("rows", "bias", "gain", "use", "more")
 
-	def __init__(self, rows, bias=None, use=None, more=None):
-		self.rows, self.bias, self.use, self.more = rows, bias, use, more
+	def __init__(self, rows, bias=None, use=None, gain=None, more=None):
+		self.rows, self.bias, self.gain, self.use, self.more = rows, bias, gain, use, more
 
 	def to(self, device, non_blocking=False):
 		def there(part):
 			return None if part is None else part.to(device, non_blocking=non_blocking)
 
-		return _Kept8(there(self.rows), there(self.bias), self.use, there(self.more))
+		return _Kept8(there(self.rows), there(self.bias), self.use, there(self.gain), there(self.more))
 
 
 def _forward8(x8, linear):
@@ -295,14 +296,16 @@ class Linear8DW(LayerDW, Linear8):
 			kernels.gemm_fp8(kept.rows, x.rows, out=self._main_grad(self.weight), epilogue=kernels.EPI_F32_ACC)
 			if self.bias is not None:
 				self._main_grad(self.bias).add_(kept.bias)
+			if kept.gain is not None:
+				self._main_grad(self.gamma).add_(kept.gain)
 			kept = kept.more
 		self.ctx["grad_output"][mb_id] = None
 		self.ctx["input"][mb_id] = None
 
 
 class NormLinear8DX(torch.autograd.Function):
-	"""(h, y) of ``NormLinear8`` (y alone without a residual).  B hands the norm's backward the product's result and h's own gradient; the
-	gain's gradient goes the way of every parameter that is no split layer's, through autograd."""
+	"""(h, y) of ``NormLinear8`` (y alone without a residual).  B hands the norm's backward the product's result, in bf16 as every layer's input
+	gradient, and h's own gradient.  The gain's gradient of a micro-batch goes through autograd, rounded, and is kept in fp32 for W."""
 
 	@staticmethod
 	def forward(ctx, x, residual, gamma, weight, bias, linear):
@@ -324,12 +327,19 @@ class NormLinear8DX(torch.autograd.Function):
 			acc = torch.zeros(gamma.shape, dtype=torch.float32, device=gamma.device)
 			dn = _backward8(_as_rows(dy), ctx.linear, ctx.use)
 			dx = kernels.norm_bwd(kernels.NORM_RMS, dn, h, gamma.detach(), stats, acc, dres=None if dh is None else _as_rows(dh)).view(ctx.in_shape)
-			dgamma = acc.to(gamma.dtype)
+			if ctx.needs_input_grad[2]:
+				dgamma = acc.to(gamma.dtype)
+				if ctx.linear.gain_in_main:
+					ctx.linear.last_grad_output.gain = acc
 		return dx, dx if ctx.added else None, dgamma, None, None, None
 
 
 class NormLinear8DW(Linear8DW, NormLinear8):
-	"""``NormLinear8`` with the split backward.  in_features: a multiple of 8, at most 8192."""
+	"""``NormLinear8`` with the split backward.  in_features: a multiple of 8, at most 8192.  The gain's gradient is summed over micro-batches in W, in
+	fp32 ``gamma.main_grad`` like the weight's and the bias's.  ``gamma.grad`` has it too, as autograd sums it in B: rounded to the parameter's
+	type after every micro-batch, until a block's ``scale_grads`` writes it from ``main_grad``."""
+
+	gain_in_main = True  # (a block says no where a module of another kind has the same parameter: only autograd's sum has that one's part)
 
 	def __init__(self, linear):
 		super().__init__(linear, linear.eps)

@@ -136,3 +136,99 @@ def test_several_backward_calls_through_one_use():
 		K.gemm_fp8(K.quant_fp8(dy, rows=False, transposed=True)[1], x8t, out=acc, epilogue=K.EPI_F32_ACC)
 		bias.add_(K.colsum_(dy, torch.zeros(72, device="cuda")))
 	assert torch.equal(layer.weight.main_grad, acc) and torch.equal(layer.bias.main_grad, bias)
+
+
+# ------------------------------------------------------------------------------------------------ the gain's gradient
+class _OneNorm(nn.Module):
+	def __init__(self, d=136, n=72, tied=False):
+		from elf_amd.models import NormLinear8, RMSNorm
+
+		super().__init__()
+		self.norm = NormLinear8(d, n, bias=False)
+		if tied:
+			self.again = RMSNorm(d)
+			self.again.weight = self.norm.gamma
+		self.tied = tied
+
+	def forward(self, a):
+		if self.tied:
+			a = self.again(a)
+		h, y = self.norm(a)
+		return (h + F.pad(y, (0, 64)),)
+
+
+def _norm_stage(tied, n_mb, T, g, variant="plain"):
+	from elf_amd.execution import AutogradStageBlock
+	from elf_amd.partitioners.utils import Signature
+	from elf_amd.scheduling import OpOptions
+
+	model = _OneNorm(tied=tied).to(torch.bfloat16)
+	with torch.no_grad():
+		model.norm.weight.copy_(torch.randn(72, 136, generator=torch.Generator().manual_seed(31)) * 0.05)
+	ref = copy.deepcopy(model).float().cuda()
+	blk = AutogradStageBlock(model, 1, [0, 1, 2], Signature(["a"], ["u"], [0], [[2]]))
+	data = [(rnd(g, T, 136), rnd(g, T, 136, by=0.1).abs()) for _ in range(n_mb)]
+	blk.zero_grad()
+	for m, (a, dy) in enumerate(data):
+		blk.input_variables[0].set(blk.input_variables[0].to_process, m, (None, a.clone()))
+		blk.forward(m)
+		out = blk.output_variables[0][0]
+		out.get(out.to_send, m)
+		out.set(out.to_process, m, (None, dy))
+		if variant == "full_bwd":
+			blk.backward_inputs(m, **{OpOptions.RECOMPUTE_ACTIVATIONS: True, OpOptions.RECOMPUTE_GRADIENTS: True})
+			blk.recompute_forward(m, **{OpOptions.SAVE: True})
+			blk.recompute_backward_inputs(m)
+		else:
+			blk.backward_inputs(m)
+		blk.input_variables[0].get(blk.input_variables[0].to_send, m)
+		blk.backward_params(m)
+	return blk, ref, data
+
+
+@pytest.mark.parametrize("variant", ["plain", "full_bwd"])
+def test_gain_over_many_micro_batches(variant):
+	"""The gain's gradient of each micro-batch is an fp32 number; their sum is that in fp32, rounded once: n half steps of fp32 and one of bf16."""
+	from elf_amd import kernels as K
+
+	n_mb, g = 96, gen(30)
+	blk, _, data = _norm_stage(False, n_mb, 40, g, variant)
+	norm = blk.model.norm
+	_, w8t = K.quant_fp8_weight(norm.weight.detach(), rows=False, transposed=True)
+	total, size, acc = torch.zeros(136, dtype=torch.float64, device="cuda"), torch.zeros(136, dtype=torch.float64, device="cuda"), torch.zeros(136, device="cuda")
+	for a, dy in data:
+		h, _, stats = K.rms_norm_fp8(a, norm.gamma.detach())
+		one = torch.zeros(136, device="cuda")
+		K.norm_bwd(K.NORM_RMS, K.gemm_fp8(K.quant_fp8(dy[:, :72].contiguous())[0], w8t), h, norm.gamma.detach(), stats, one)
+		total, size = total + one.double(), size + one.double().abs()
+		acc.add_(one)
+	assert torch.equal(norm.gamma.main_grad, acc)
+	off = n_mb * 2.0**-24 * size
+	assert ((acc.double() - total).abs() <= off).all()
+	blk.scale_grads(n_mb)
+	assert norm.gamma.grad.dtype == torch.bfloat16
+	assert ((norm.gamma.grad.double() - total / n_mb).abs() <= 2.0**-8 * (total.abs() / n_mb) + 2 * off / n_mb).all()
+	blk.zero_grad()
+	assert norm.gamma.grad is None and not norm.gamma.main_grad.any()
+
+
+def test_gain_that_another_module_shares():
+	"""A plain norm with the same parameter: both parts of its gradient count."""
+	blk, ref, data = _norm_stage(True, 3, 40, gen(32))
+	for a, dy in data:
+		ref(a.float().requires_grad_(True))[0].backward(dy.float())
+	blk.scale_grads(3)
+	near(blk.model.norm.gamma.grad, ref.norm.gamma.grad / 3, 0.06, "gain")
+
+
+def test_frozen_gain():
+	from elf_amd.models import NormLinear8
+
+	g = gen(33)
+	layer = make(NormLinear8, 64, 48, False, E4M3, g)
+	layer.gamma.requires_grad_(False)
+	h, y = layer(rnd(g, 20, 64).requires_grad_(True))
+	y.backward(rnd(g, 20, 48))
+	moved(layer, 0)
+	layer.backward(0)
+	assert layer.gamma.grad is None and getattr(layer.gamma, "main_grad", None) is None
