@@ -202,10 +202,21 @@ class LinearDW(LayerDW, nn.Linear):
 LinearDW.register_dx_function(LinearDX)
 
 # ------------------------------------------------------------------------------------------------ 8 bits
+class _Use:
+	"""One forward call of a layer in 8 bits.  ``lost``: the layer was called again before its input was moved, so W would multiply this call's
+	output gradient with the other's input.  A checkpoint that runs the forward again, within a backward pass (``task``), loses nothing: it
+	stores the input that was there."""
+
+	__slots__ = ("task", "lost")
+
+	def __init__(self):
+		self.task, self.lost = torch._C._current_graph_task_id(), False
+
+
 class _Kept8:
 	"""What a layer in 8 bits keeps of a micro-batch: its input or its output gradient along the tokens (``kernels.Fp8Rows`` of the
 	transpose, half of the bf16 bytes), and of an output gradient its sum over the tokens where there is a bias and the gradient of the gain where
-	there is a norm, both in fp32.  ``use``: the forward call that an output gradient belongs to; ``more``: what came before it of the same call (a
+	there is a norm, both in fp32.  ``use``: the forward call it belongs to; ``more``: what came before it of the same call (a
 	stage goes back from its outputs one after the other)."""
 
 	__slots__ = ("rows", "bias", "gain", "use", "more")
@@ -246,8 +257,7 @@ class Linear8DX(torch.autograd.Function):
 	@staticmethod
 	def forward(ctx, input, weight, bias, linear):
 		x8, x8t = kernels.quant_fp8(_as_rows(input.detach()), transposed=True)
-		linear._store_input8(x8t)
-		ctx.linear, ctx.in_shape, ctx.use = linear, input.shape, object()
+		ctx.linear, ctx.in_shape, ctx.use = linear, input.shape, linear._store_input8(x8t)
 		ctx.save_for_backward(x8t.memory)  # read again in B, so that torch.utils.checkpoint runs the forward again
 		return _forward8(x8, linear).view(*input.shape[:-1], weight.shape[0])
 
@@ -274,7 +284,11 @@ class Linear8DW(LayerDW, Linear8):
 			raise _lib.ElfStageError(f"{type(self).__name__}: bf16 tensors on the GPU only (input {x.dtype} on {x.device}, weight {self.weight.dtype} on {self.weight.device})")
 
 	def _store_input8(self, rows):
-		self.__dict__["last_input"] = _Kept8(rows)
+		last, use = self.last_input, _Use()
+		if last is not None and last.use.task == use.task:
+			last.use.lost = True
+		self.__dict__["last_input"] = _Kept8(rows, use=use)
+		return use
 
 	def _store_grad_output(self, kept):
 		last = getattr(self, "last_grad_output", None)
@@ -290,8 +304,10 @@ class Linear8DW(LayerDW, Linear8):
 		return Linear8DX.apply(x, self.weight, self.bias, self)
 
 	def backward(self, mb_id):
-		"""W: main_grad += dY^T X (fp32) from the two 8-bit matrices, bias main_grad += the sum that B left; drops the stash."""
+		"""W: main_grad += dY^T X (fp32) from the two 8-bit matrices, the bias's and the gain's += what B left; drops the stash."""
 		kept, x = self.ctx["grad_output"][mb_id], self.ctx["input"][mb_id]
+		if kept.use.lost:
+			raise _lib.ElfStageError(f"{type(self).__name__}: the layer was used several times in one forward, or again before its input was moved: what is kept is not the input of the use that has a gradient")
 		while kept is not None:
 			kernels.gemm_fp8(kept.rows, x.rows, out=self._main_grad(self.weight), epilogue=kernels.EPI_F32_ACC)
 			if self.bias is not None:
@@ -311,8 +327,7 @@ class NormLinear8DX(torch.autograd.Function):
 	def forward(ctx, x, residual, gamma, weight, bias, linear):
 		rows = None if residual is None else _as_rows(residual.detach())
 		h, n8, stats = kernels.rms_norm_fp8(_as_rows(x.detach()), gamma.detach(), residual=rows, eps=linear.eps)
-		linear._store_input8(kernels.transpose_fp8(n8))
-		ctx.linear, ctx.in_shape, ctx.use, ctx.added = linear, x.shape, object(), residual is not None
+		ctx.linear, ctx.in_shape, ctx.use, ctx.added = linear, x.shape, linear._store_input8(kernels.transpose_fp8(n8)), residual is not None
 		ctx.set_materialize_grads(False)
 		y = _forward8(n8, linear).view(*x.shape[:-1], weight.shape[0])
 		ctx.save_for_backward(h, stats, gamma)

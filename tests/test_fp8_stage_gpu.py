@@ -232,3 +232,54 @@ def test_frozen_gain():
 	moved(layer, 0)
 	layer.backward(0)
 	assert layer.gamma.grad is None and getattr(layer.gamma, "main_grad", None) is None
+
+
+# ------------------------------------------------------------------------------------------------ one use in a forward
+@pytest.mark.parametrize("which", [0, 1])
+def test_only_one_of_two_uses_has_a_gradient(which):
+	"""W has the input of the last use: it refuses a gradient of the first, and is right with one of the last."""
+	from elf_amd import kernels as K
+	from elf_amd._lib import ElfStageError
+	from elf_amd.models import Linear8
+
+	g = gen(40)
+	layer = make(Linear8, 72, 48, False, E4M3, g)
+	xs, dy = [rnd(g, 20, 72).requires_grad_(True) for _ in range(2)], rnd(g, 20, 48)
+	ys = [layer(x) for x in xs]
+	ys[which].backward(dy)
+	moved(layer, 0)
+	if which == 0:
+		with pytest.raises(ElfStageError, match="several times"):
+			layer.backward(0)
+		return
+	layer.backward(0)
+	x8t, dy8t = (K.quant_fp8(t, rows=False, transposed=True)[1] for t in (xs[1].detach(), dy))
+	assert torch.equal(layer.weight.main_grad, K.gemm_fp8(dy8t, x8t, epilogue=K.EPI_F32_STORE))
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_outside_of_a_stage(reentrant):
+	"""The forward that a checkpoint runs again is no second use; neither is a call without gradients before or after the step."""
+	from elf_amd.models import Linear8
+	from torch.utils.checkpoint import checkpoint
+
+	g = gen(41)
+	layers = nn.Sequential(make(Linear8, 72, 48, True, E4M3, g), nn.Tanh(), make(Linear8, 48, 72, False, E5M2, g))
+	x, dy = rnd(g, 20, 72), rnd(g, 20, 72)
+
+	def step(call):
+		a = x.clone().requires_grad_(True)
+		with torch.no_grad():
+			layers(a)
+		y = call(a)
+		y.backward(dy)
+		for layer in (layers[0], layers[2]):
+			layer.weight.main_grad = None
+			moved(layer, 0)
+			layer.backward(0)
+		with torch.no_grad():
+			layers(a)
+		return y.detach(), a.grad, layers[0].weight.main_grad, layers[2].weight.main_grad
+
+	for got, want in zip(step(lambda a: checkpoint(layers, a, use_reentrant=reentrant)), step(layers)):
+		assert torch.equal(got, want)
