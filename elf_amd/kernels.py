@@ -505,9 +505,9 @@ def dequant_fp8(a):
 	return out
 
 
-def rms_norm_fp8(x, gamma, residual=None, eps=1e-5, dtype=torch.float8_e4m3fn):
-	"""(h, y, stats): h = x + residual (bf16; x itself without one), y = RMSNorm(h) * gamma as ``Fp8Rows``, stats [T, 2] for
-	``norm_bwd(NORM_RMS, dy, h, gamma, stats, dgamma, dres=dh)``, whose result is the gradient of x and of the residual."""
+def rms_norm_fp8(x, gamma, residual=None, eps=1e-5, dtype=torch.float8_e4m3fn, h=None):
+	"""(h, y, stats): h = x + residual (bf16; x itself without one; in the memory of ``h`` where that is given, which may be x or the
+	residual), y = RMSNorm(h) * gamma as ``Fp8Rows``, stats [T, 2] for ``norm_bwd(NORM_RMS, dy, h, gamma, stats, dgamma, dres=dh)``, whose result is the gradient of x and of the residual."""
 	fmt, shape, device, index = _format(dtype, "rms_norm_fp8"), x.shape, x.device, x.get_device()
 	_here(index, device, "rms_norm_fp8")
 	if x.dtype != torch.bfloat16 or len(shape) != 2 or not x.is_contiguous():
@@ -515,11 +515,19 @@ def rms_norm_fp8(x, gamma, residual=None, eps=1e-5, dtype=torch.float8_e4m3fn):
 	T, d = shape
 	if gamma.dtype != torch.bfloat16 or gamma.numel() != d or not gamma.is_contiguous() or gamma.get_device() != index:
 		raise _lib.ElfStageError(f"rms_norm_fp8: gamma must hold x's {d} columns in bfloat16 on {device}, got {gamma.dtype} {tuple(gamma.shape)} on {gamma.device}")
-	h, r = x, None
-	if residual is not None:
+	r = None
+	if residual is None:
+		if h is not None:
+			raise _lib.ElfStageError("rms_norm_fp8: without a residual h is x itself")
+		h = x
+	else:
 		if residual.shape != shape or residual.dtype != torch.bfloat16 or not residual.is_contiguous() or residual.get_device() != index:
 			raise _lib.ElfStageError(f"rms_norm_fp8: the residual must be dense and of x's shape {tuple(shape)} in bfloat16 on {device}, got {residual.dtype} {tuple(residual.shape)} on {residual.device}")
-		h, r = torch.empty(shape, dtype=torch.bfloat16, device=device), residual.data_ptr()
+		r = residual.data_ptr()
+		if h is None:
+			h = torch.empty(shape, dtype=torch.bfloat16, device=device)
+		elif h.shape != shape or h.dtype != torch.bfloat16 or not h.is_contiguous() or h.get_device() != index:
+			raise _lib.ElfStageError(f"rms_norm_fp8: h must be dense and of x's shape {tuple(shape)} in bfloat16 on {device}, got {h.dtype} {tuple(h.shape)} on {h.device}")
 	y = Fp8Rows.empty(T, d, dtype, device)
 	stats = torch.empty((T, 2), dtype=torch.float32, device=device)
 	rc = _lib.load().elf_rms_norm_fp8(x.data_ptr(), r, gamma.data_ptr(), h.data_ptr(), *y._args, stats.data_ptr(), T, d, eps, fmt, _stream())

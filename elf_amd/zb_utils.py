@@ -231,11 +231,18 @@ class _Kept8:
 		return _Kept8(there(self.rows), there(self.bias), self.use, there(self.gain), there(self.more))
 
 
-def _forward8(x8, linear):
+def _forward8(x8, linear, lead):
+	"""[*lead, out_features] of rows in 8 bits, in memory of its own: a view would keep users from writing into it in place."""
 	w8, _ = kernels.quant_fp8_weight(linear.weight.detach())
+	y = rows = None
+	if len(lead) != 1:
+		y = torch.empty((*lead, linear.weight.shape[0]), dtype=torch.bfloat16, device=linear.weight.device)
+		rows = y.view(-1, y.shape[-1])
 	if linear.bias is None:
-		return kernels.gemm_fp8(x8, w8)
-	return kernels.gemm_fp8(x8, w8, epilogue=kernels.EPI_BF16_RESID, residual=linear.bias.detach(), residual_ld=0)
+		rows = kernels.gemm_fp8(x8, w8, out=rows)
+	else:
+		rows = kernels.gemm_fp8(x8, w8, out=rows, epilogue=kernels.EPI_BF16_RESID, residual=linear.bias.detach(), residual_ld=0)
+	return rows if y is None else y
 
 
 def _backward8(go, linear, use):
@@ -259,7 +266,7 @@ class Linear8DX(torch.autograd.Function):
 		x8, x8t = kernels.quant_fp8(_as_rows(input.detach()), transposed=True)
 		ctx.linear, ctx.in_shape, ctx.use = linear, input.shape, linear._store_input8(x8t)
 		ctx.save_for_backward(x8t.memory)  # read again in B, so that torch.utils.checkpoint runs the forward again
-		return _forward8(x8, linear).view(*input.shape[:-1], weight.shape[0])
+		return _forward8(x8, linear, input.shape[:-1])
 
 	@staticmethod
 	def backward(ctx, grad_output):
@@ -320,18 +327,20 @@ class Linear8DW(LayerDW, Linear8):
 
 
 class NormLinear8DX(torch.autograd.Function):
-	"""(h, y) of ``NormLinear8`` (y alone without a residual).  B hands the norm's backward the product's result, in bf16 as every layer's input
+	"""(h, y) of ``NormLinear8`` (y alone without a residual).  B reads h again: where h was written in place, autograd refuses.  It hands the norm's backward the product's result, in bf16 as every layer's input
 	gradient, and h's own gradient.  The gain's gradient of a micro-batch goes through autograd, rounded, and is kept in fp32 for W."""
 
 	@staticmethod
 	def forward(ctx, x, residual, gamma, weight, bias, linear):
-		rows = None if residual is None else _as_rows(residual.detach())
-		h, n8, stats = kernels.rms_norm_fp8(_as_rows(x.detach()), gamma.detach(), residual=rows, eps=linear.eps)
+		rows, added, h = _as_rows(x.detach()), None, None
+		if residual is not None:
+			added, h = _as_rows(residual.detach()), torch.empty(x.shape, dtype=x.dtype, device=x.device)
+		h_rows, n8, stats = kernels.rms_norm_fp8(rows, gamma.detach(), residual=added, eps=linear.eps, h=None if h is None else h.view(rows.shape))
 		ctx.linear, ctx.in_shape, ctx.use, ctx.added = linear, x.shape, linear._store_input8(kernels.transpose_fp8(n8)), residual is not None
 		ctx.set_materialize_grads(False)
-		y = _forward8(n8, linear).view(*x.shape[:-1], weight.shape[0])
-		ctx.save_for_backward(h, stats, gamma)
-		return (h.view(x.shape), y) if ctx.added else y
+		y = _forward8(n8, linear, x.shape[:-1])
+		ctx.save_for_backward(h_rows if h is None else h, stats, gamma)
+		return (h, y) if ctx.added else y
 
 	@staticmethod
 	def backward(ctx, *grads):
@@ -341,7 +350,7 @@ class NormLinear8DX(torch.autograd.Function):
 		if dy is not None:
 			acc = torch.zeros(gamma.shape, dtype=torch.float32, device=gamma.device)
 			dn = _backward8(_as_rows(dy), ctx.linear, ctx.use)
-			dx = kernels.norm_bwd(kernels.NORM_RMS, dn, h, gamma.detach(), stats, acc, dres=None if dh is None else _as_rows(dh)).view(ctx.in_shape)
+			dx = kernels.norm_bwd(kernels.NORM_RMS, dn, _as_rows(h), gamma.detach(), stats, acc, dres=None if dh is None else _as_rows(dh)).view(ctx.in_shape)
 			if ctx.needs_input_grad[2]:
 				dgamma = acc.to(gamma.dtype)
 				if ctx.linear.gain_in_main:

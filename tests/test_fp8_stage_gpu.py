@@ -283,3 +283,61 @@ def test_checkpointed_outside_of_a_stage(reentrant):
 
 	for got, want in zip(step(lambda a: checkpoint(layers, a, use_reentrant=reentrant)), step(layers)):
 		assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------------------------ outputs written in place
+@pytest.mark.parametrize("shape", [(72,), (20, 72), (2, 10, 72), (2, 3, 4, 72)])
+def test_outputs_are_written_in_place(shape):
+	"""``nn.ReLU(inplace=True)`` and the like behind a product give what they give on a copy."""
+	from elf_amd.models import Linear8, NormLinear8
+
+	g = gen(50)
+	linear, norm = make(Linear8, 72, 48, True, E4M3, g), make(NormLinear8, 72, 48, True, E4M3, g)
+	x, r, dy = rnd(g, *shape), rnd(g, *shape), rnd(g, *shape[:-1], 48)
+
+	def step(call, change):
+		a, b = x.clone().requires_grad_(True), r.clone().requires_grad_(True)
+		y = change(call(a, b))
+		y.backward(dy)
+		linear.clear()
+		norm.clear()
+		return y.detach(), a.grad
+
+	for call in (lambda a, b: linear(a), lambda a, b: norm(a)[1], lambda a, b: norm(a, b)[1]):
+		for got, want in zip(step(call, lambda y: y.mul_(2).relu_()), step(call, lambda y: y.clone().mul_(2).relu_())):
+			assert got.shape == want.shape and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("shape", [(20, 72), (2, 10, 72)])
+def test_residual_stream_written_in_place_is_refused(shape):
+	"""B reads h: autograd notices that it is no longer there, whether h is the sum or the input itself."""
+	from elf_amd.models import NormLinear8
+
+	g = gen(51)
+	norm = make(NormLinear8, 72, 72, False, E4M3, g)
+	for inputs in ([rnd(g, *shape), rnd(g, *shape)], [rnd(g, *shape)]):
+		h, y = norm(*[(t.requires_grad_(True) * 1) for t in inputs])
+		h += y
+		with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+			h.sum().backward()
+		norm.clear()
+
+
+def test_norm_into_given_memory():
+	from elf_amd import kernels as K
+	from elf_amd._lib import ElfStageError
+
+	g = gen(52)
+	x, r, gamma = rnd(g, 20, 72), rnd(g, 20, 72), 1 + rnd(g, 72, by=0.1)
+	want = K.rms_norm_fp8(x, gamma, residual=r)
+	for h in (torch.full_like(x, 3.0), x.clone(), r.clone()):
+		into = [x.clone(), r.clone()]
+		for i, t in enumerate((x, r)):
+			if torch.equal(h, t):
+				into[i] = h
+		got = K.rms_norm_fp8(into[0], gamma, residual=into[1], h=h)
+		assert got[0] is h and torch.equal(h, want[0]) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip((got[1].q, got[1].scale), (want[1].q, want[1].scale))) and torch.equal(got[2], want[2])
+	with pytest.raises(ElfStageError, match="h must be dense"):
+		K.rms_norm_fp8(x, gamma, residual=r, h=torch.empty(20, 80, dtype=torch.bfloat16, device="cuda")[:, :72])
+	with pytest.raises(ElfStageError, match="x itself"):
+		K.rms_norm_fp8(x, gamma, h=torch.empty_like(x))
