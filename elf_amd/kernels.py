@@ -395,6 +395,18 @@ class Fp8Rows:
 		blocks = -(-cols // FP8_BLOCK)
 		return Fp8Rows._of(torch.empty(rows * blocks * FP8_BLOCK + blocks * (-(-rows // 16) * 16), dtype=torch.uint8, device=device), rows, cols, dtype)
 
+	def __reduce__(self):
+		"""Copies and pickles are made anew from their tensors, as bytes (``torch.save`` does not know the scales' type): the pointers are this
+		matrix's only."""
+		rows, cols = self.shape
+		if self._buf is not None:
+			return Fp8Rows._of, (self._buf, rows, cols, self.dtype)
+		return Fp8Rows._of_bytes, (self._q.view(torch.uint8), self._scale.view(torch.uint8), cols, self.dtype)
+
+	@staticmethod
+	def _of_bytes(q, scale, cols, dtype):
+		return Fp8Rows(q.view(dtype), scale.view(torch.float8_e8m0fnu), cols)
+
 	@property
 	def cols(self):
 		return self.shape[1]
