@@ -47,11 +47,12 @@ __device__ __forceinline__ void load16(const PackArgs& g, int64_t row, int64_t c
 		}
 	} else {
 		const u32x4 w = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(g.x) + row * g.ldx + col);
-		const int e = (int)g.sx[(col >> 7) * g.ldsx + row] - 127 - UP;
+		const uint32_t byte = g.sx[(col >> 7) * g.ldsx + row];
+		const int e = (int)byte - 127 - UP;
 #pragma unroll
 		for (int i = 0; i < 4; i++) {
 			float u[4];
-			fp8_unpack4<SRC>(w[i], u);
+			fp8_unpack4<SRC>(fp8_or_nan(w[i], byte), u);
 #pragma unroll
 			for (int j = 0; j < 4; j++) v[i * 4 + j] = col + i * 4 + j < g.C ? __builtin_ldexpf(u[j], e) : 0.f;
 		}
@@ -164,22 +165,22 @@ __global__ __launch_bounds__(256) void dequant_kernel(PackArgs g, bf16_t* out, i
 	const int64_t cb = blockIdx.x % g.col_blocks, rb = blockIdx.x / g.col_blocks;
 	const int64_t col = cb * 128 + c * 8;
 	u32x2 raw[8];
-	int e[8];
+	uint32_t byte[8];
 #pragma unroll
 	for (int p = 0; p < 8; p++) {
 		const int64_t row = min(rb * 128 + p * 16 + r, g.T - 1);
 		raw[p] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint8_t*>(g.x) + row * g.ldx + col);
-		e[p] = (int)g.sx[cb * g.ldsx + row] - 127;
+		byte[p] = g.sx[cb * g.ldsx + row];
 	}
 #pragma unroll
 	for (int p = 0; p < 8; p++) {
 		const int64_t row = rb * 128 + p * 16 + r;
 		float u[2][4];
-		fp8_unpack4<FMT>(raw[p][0], u[0]);
-		fp8_unpack4<FMT>(raw[p][1], u[1]);
+		fp8_unpack4<FMT>(fp8_or_nan(raw[p][0], byte[p]), u[0]);
+		fp8_unpack4<FMT>(fp8_or_nan(raw[p][1], byte[p]), u[1]);
 		bf16x8 o;
 #pragma unroll
-		for (int j = 0; j < 8; j++) o[j] = (bf16_t)__builtin_ldexpf(u[j >> 2][j & 3], e[p]);  // exact (2^128 becomes an infinity)
+		for (int j = 0; j < 8; j++) o[j] = (bf16_t)__builtin_ldexpf(u[j >> 2][j & 3], (int)byte[p] - 127);  // exact (2^128 becomes an infinity)
 		const u32x4 v = __builtin_bit_cast(u32x4, o);
 		uint32_t next = 0;
 		if (g.between) next = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[0], 0x101, 0xf, 0xf, false);  // row_shl 1: the lane behind

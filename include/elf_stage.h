@@ -184,7 +184,7 @@ int elf_swiglu_bwd(const void* dh, const void* gu, void* dgu, int64_t T, int F, 
  *
  * A matrix of R rows and C columns in 8 bits is q[R, ld] (fmt 0: e4m3, 1: e5m2; one byte a value, ld at least C rounded up to 128,
  * the columns from C to that zero) and s[blocks, lds] (blocks = C / 128 rounded up; one byte E8M0 a block: values of row r and
- * columns 128 b .. 128 b + 127 are q times 2^(s[b * lds + r] - 127)).  ld and lds are multiples of 16, q and s 16-byte aligned,
+ * columns 128 b .. 128 b + 127 are q times 2^(s[b * lds + r] - 127), and no numbers where that byte is 255).  ld and lds are multiples of 16, q and s 16-byte aligned,
  * lds >= R; s is read up to R rounded up to 4.  A block's scale is the smallest power of two, not below 2^-126, for which its
  * largest finite magnitude is at most the type's largest number (448, 57344), and 1 where there is none; values are rounded to
  * nearest, ties to even.  NaN stays NaN, infinities become NaN in e4m3 and stay in e5m2; neither has a say in the scale.
@@ -193,7 +193,8 @@ int elf_swiglu_bwd(const void* dh, const void* gu, void* dgu, int64_t T, int F, 
  * matrix of the transpose, [C, T]) or both, from one read of x; q or qt is NULL where that one is not wanted.  square != 0 (e4m3
  * only; weights): one scale for each 128 x 128 values, so that both layouts hold the same numbers.
  * elf_transpose_fp8: the transpose of a matrix in 8 bits, in 8 bits.  Scales are powers of two, so the values stay as they are, but
- * for those below 2^-13 (e5m2: 2^-28) of the largest of their new block, which are rounded once more.
+ * for those below 2^-13 (e5m2: 2^-28) of the largest of their new block, which are rounded once more.  Scales go up to 2^121 (e5m2: 2^114; the
+ * library's own end at 2^120 and 2^113): values of larger ones may become infinities.
  * elf_dequant_fp8: the values as bf16 (exact: every value of either type times any scale from 2^-117 on is a bf16 number, but for 2^128,
  * to which magnitudes from 1.9375 2^127 on are rounded and which comes back as an infinity). */
 int elf_quant_fp8(const void* x, int64_t ldx, int64_t T, int64_t C, int fmt, int square, void* q, int64_t ldq, void* s, int64_t lds,
