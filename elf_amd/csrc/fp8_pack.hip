@@ -199,11 +199,11 @@ __global__ __launch_bounds__(256) void dequant_kernel(PackArgs g, bf16_t* out, i
 
 // h = x + residual (rounded to bf16: what the residual stream keeps is what is normalized), y = h * rsqrt(mean(h^2) + eps) * gamma, and y goes
 // into 8 bits straight from fp32: it is rounded once.  One wave a row, or four where the row is longer than 2048; a thread holds chunks of 8
-// values, a block of 128 is 16 neighbouring lanes.
+// values, a block of 128 is 16 neighbouring lanes.  h may be x's or the residual's memory: a thread reads all of its chunks before it writes one.
 template <int NCH, int WPR, int FMT>
-__global__ __launch_bounds__(256) void rms_norm_fp8_kernel(const bf16_t* __restrict__ x, const bf16_t* __restrict__ residual, const bf16_t* __restrict__ gamma,
-                                                           bf16_t* __restrict__ h, uint8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ s, int64_t lds,
-                                                           float2* __restrict__ stats, int64_t T, int d, float eps) {
+__global__ __launch_bounds__(256) void rms_norm_fp8_kernel(const bf16_t* x, const bf16_t* residual, const bf16_t* __restrict__ gamma, bf16_t* h,
+                                                           uint8_t* __restrict__ q, int64_t ldq, uint8_t* __restrict__ s, int64_t lds, float2* __restrict__ stats,
+                                                           int64_t T, int d, float eps) {
 	__shared__ float red[4];
 	const int wave = threadIdx.x >> 6;
 	const int tr = WPR == 1 ? (threadIdx.x & 63) : threadIdx.x;
@@ -211,6 +211,15 @@ __global__ __launch_bounds__(256) void rms_norm_fp8_kernel(const bf16_t* __restr
 	const int64_t row = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
 	if (row >= T) return;  // whole waves (WPR 1) or whole workgroups
 	const int nchunks = d >> 3, padded = (d + 127) / 128 * 16;
+	bf16x8 o[NCH], r[NCH];
+#pragma unroll
+	for (int i = 0; i < NCH; i++) {
+		const int ch = tr + i * TPR;
+		if (ch < nchunks) {
+			o[i] = *reinterpret_cast<const bf16x8*>(x + row * d + ch * 8);
+			if (residual) r[i] = *reinterpret_cast<const bf16x8*>(residual + row * d + ch * 8);
+		}
+	}
 	float v[NCH][8];
 	float ss = 0.f;
 #pragma unroll
@@ -219,17 +228,14 @@ __global__ __launch_bounds__(256) void rms_norm_fp8_kernel(const bf16_t* __restr
 #pragma unroll
 		for (int j = 0; j < 8; j++) v[i][j] = 0.f;
 		if (ch < nchunks) {
-			const bf16x8 a = *reinterpret_cast<const bf16x8*>(x + row * d + ch * 8);
-			bf16x8 o = a;
 			if (residual) {
-				const bf16x8 b = *reinterpret_cast<const bf16x8*>(residual + row * d + ch * 8);
 #pragma unroll
-				for (int j = 0; j < 8; j++) o[j] = (bf16_t)((float)a[j] + (float)b[j]);
-				*reinterpret_cast<bf16x8*>(h + row * d + ch * 8) = o;
+				for (int j = 0; j < 8; j++) o[i][j] = (bf16_t)((float)o[i][j] + (float)r[i][j]);
+				*reinterpret_cast<bf16x8*>(h + row * d + ch * 8) = o[i];
 			}
 #pragma unroll
 			for (int j = 0; j < 8; j++) {
-				v[i][j] = (float)o[j];
+				v[i][j] = (float)o[i][j];
 				ss += v[i][j] * v[i][j];
 			}
 		}

@@ -341,3 +341,17 @@ def test_norm_into_given_memory():
 		K.rms_norm_fp8(x, gamma, residual=r, h=torch.empty(20, 80, dtype=torch.bfloat16, device="cuda")[:, :72])
 	with pytest.raises(ElfStageError, match="x itself"):
 		K.rms_norm_fp8(x, gamma, h=torch.empty_like(x))
+
+
+@pytest.mark.parametrize("over", ["x", "residual"])
+@pytest.mark.parametrize("T,d", [(5, 72), (7, 520), (130, 1600), (9, 4096), (67, 4104), (300, 8192)])
+def test_norm_over_its_inputs(T, d, over):
+	"""h in the memory of x or of the residual, at every number of chunks a thread holds."""
+	from elf_amd import kernels as K
+
+	g = gen(T + d)
+	x, r, gamma = rnd(g, T, d), rnd(g, T, d), 1 + rnd(g, d, by=0.1)
+	want = K.rms_norm_fp8(x, gamma, residual=r)
+	got = K.rms_norm_fp8(x, gamma, residual=r, h=x if over == "x" else r)
+	assert got[0] is (x if over == "x" else r) and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+	assert torch.equal(got[1].q.view(torch.uint8), want[1].q.view(torch.uint8)) and torch.equal(got[1].scale.view(torch.uint8), want[1].scale.view(torch.uint8))
