@@ -52,6 +52,8 @@ __device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t top_bits) {
 __device__ __forceinline__ float fp8_inverse(uint32_t byte) { return __builtin_bit_cast(float, (254u - byte) << 23); }
 // What a block holds whose scale is not a number (byte 255): NaN in either type.
 __device__ __forceinline__ uint32_t fp8_or_nan(uint32_t w, uint32_t scale_byte) { return scale_byte == 255u ? 0x7f7f7f7fu : w; }
+// The scale itself, of any byte: 2^-127 is a subnormal number, 255 is not a number.
+__device__ __forceinline__ float fp8_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23 | (((byte + 1u) & 0xffu) < 2u ? 0x400000u : 0u)); }
 // |v| as fp32 bits, 0 where v is no finite number
 __device__ __forceinline__ uint32_t fp8_magnitude(float v) {
 	const uint32_t a = __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;

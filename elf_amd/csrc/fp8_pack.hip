@@ -176,11 +176,12 @@ __global__ __launch_bounds__(256) void dequant_kernel(PackArgs g, bf16_t* out, i
 	for (int p = 0; p < 8; p++) {
 		const int64_t row = rb * 128 + p * 16 + r;
 		float u[2][4];
-		fp8_unpack4<FMT>(fp8_or_nan(raw[p][0], byte[p]), u[0]);
-		fp8_unpack4<FMT>(fp8_or_nan(raw[p][1], byte[p]), u[1]);
+		fp8_unpack4<FMT>(raw[p][0], u[0]);
+		fp8_unpack4<FMT>(raw[p][1], u[1]);
+		const float scale = fp8_scale(byte[p]);
 		bf16x8 o;
 #pragma unroll
-		for (int j = 0; j < 8; j++) o[j] = (bf16_t)__builtin_ldexpf(u[j >> 2][j & 3], (int)byte[p] - 127);  // exact (2^128 becomes an infinity)
+		for (int j = 0; j < 8; j++) o[j] = (bf16_t)(u[j >> 2][j & 3] * scale);  // exact (2^128 becomes an infinity)
 		const u32x4 v = __builtin_bit_cast(u32x4, o);
 		uint32_t next = 0;
 		if (g.between) next = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[0], 0x101, 0xf, 0xf, false);  // row_shl 1: the lane behind
