@@ -170,10 +170,10 @@ __device__ __forceinline__ u32x4 buffer_of(const uint8_t* base, uint32_t bytes) 
 __device__ __forceinline__ uint32_t scale_bytes(int rows) { return (uint32_t)min(256, (rows + 3) & ~3); }
 template <int IMM>
 __device__ __forceinline__ void load_lds16(const u32x4& buf, uint32_t off, uint32_t lds) {
-	asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(buf), "n"(IMM) : "memory", "scc");
+	asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(buf), "n"(IMM) : "memory", "m0", "scc");
 }
 __device__ __forceinline__ void load_lds4(const u32x4& buf, uint32_t off, uint32_t lds) {
-	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(buf) : "memory");
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(buf) : "memory", "m0");
 }
 
 // Places of the 16-byte chunks of a row's 128 bytes in LDS, as a function of the row: chunk c lies at c ^ swz(row).  Token rows are read 16
