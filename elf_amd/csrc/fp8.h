@@ -17,13 +17,6 @@ namespace elf {
 enum Fp8Format { FP8_E4M3 = 0, FP8_E5M2 = 1 };
 constexpr int FP8_BLOCK = 128;
 
-struct Fp8View {
-	const uint8_t* q;
-	int64_t ld;
-	const uint8_t* s;
-	int64_t lds;
-};
-
 // x [T, C] (bf16, rows ldx apart) -> its rows in 8 bits (q, s) and / or its columns (qt [C, ldqt], st); square: one scale for 128 x 128.
 int quant_fp8(const void* x, int64_t ldx, int64_t T, int64_t C, int fmt, int square, void* q, int64_t ldq, void* s, int64_t lds, void* qt, int64_t ldqt, void* st,
               int64_t ldst, hipStream_t stream);

@@ -7,26 +7,26 @@ namespace fp8 {
 
 constexpr int64_t MOST = (int64_t(1) << 31) - 512;  // M, N and K
 
-// Four waves, 2 x 2, each (BM / 2) x (BN / 2) of the tile; a ring of NS K slices in LDS, filled by direct-to-LDS loads NS - 1 slices ahead.
-// Bound: the chain barrier -> fragment reads -> MFMAs of a slice, 0.32 us of 64 x 64 x 128 and 0.45 for two workgroups of a compute unit (four
+// 64 x 64 tiles: four waves, 2 x 2, each 32 x 32; a ring of four K slices in LDS, filled by direct-to-LDS loads three slices ahead.
+// Bound: the chain barrier -> fragment reads -> MFMAs of a slice, 0.32 us and 0.45 for two workgroups of a compute unit (four
 // slices in LDS; two slices 0.53 and 0.54, eight 0.38).
 // A slice of an operand is its rows' 128 bytes of one block, 16-byte chunk c of row r in place c ^ f(r) so that the 16 lanes of a
 // fragment read meet 16 different bank groups, and one scale byte a row.  Rows behind the matrix are zeros.
 // A lane's share of a fragment is the chunks q and q + 4 of its row, q = lane / 16: the order of k within a block is free, as long as both
 // operands have the same.
-template <int BM, int BN, int NS>
 struct Ring {
+	static constexpr int BM = 64, BN = 64, NS = 4;
 	static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
 	static constexpr int SCALES = 4 * 256;  // a dword per thread
 	static constexpr int STAGE = A_BYTES + B_BYTES + SCALES;
 	static constexpr int BYTES = NS * STAGE;
 };
 
-template <int BM, int BN, int NS, int FMT>
+template <int FMT>
 __global__ __launch_bounds__(256) void gemm_kernel(Args g) {
-	using Rg = Ring<BM, BN, NS>;
+	constexpr int BM = Ring::BM, BN = Ring::BN, NS = Ring::NS;
 	constexpr int RA = BM / 32, RB = BN / 32;  // 16-row fragments of a wave
-	constexpr int LA = Rg::A_BYTES / 4096, LB = Rg::B_BYTES / 4096;
+	constexpr int LA = Ring::A_BYTES / 4096, LB = Ring::B_BYTES / 4096;
 	extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
 	const int tid = threadIdx.x, lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -62,11 +62,11 @@ __global__ __launch_bounds__(256) void gemm_kernel(Args g) {
 	// slice kt into a stage; one behind the last is fetched from the last: the count of loads in flight stays the same, and nobody reads it
 	auto fetch = [&](int kt, int stage) {
 		kt = min(kt, nk - 1);
-		const uint32_t at = lds + (uint32_t)stage * Rg::STAGE;
+		const uint32_t at = lds + (uint32_t)stage * Ring::STAGE;
 		const u32x4 ab = buffer_of(ap + (int64_t)kt * BK, a_bytes), bb = buffer_of(bp + (int64_t)kt * BK, b_bytes);
 		static_for<LA>([&](auto ic) { load_lds16<decltype(ic)::value * 1024>(ab, aoff[decltype(ic)::value], at + wave * (LA * 1024)); });
-		static_for<LB>([&](auto ic) { load_lds16<decltype(ic)::value * 1024>(bb, boff[decltype(ic)::value], at + Rg::A_BYTES + wave * (LB * 1024)); });
-		load_lds4(buffer_of(sp + kt * s_step, s_bytes), lane * 4, at + Rg::A_BYTES + Rg::B_BYTES + wave * 256);
+		static_for<LB>([&](auto ic) { load_lds16<decltype(ic)::value * 1024>(bb, boff[decltype(ic)::value], at + Ring::A_BYTES + wave * (LB * 1024)); });
+		load_lds4(buffer_of(sp + kt * s_step, s_bytes), lane * 4, at + Ring::A_BYTES + Ring::B_BYTES + wave * 256);
 	};
 
 	f32x4 acc[RA][RB];
@@ -83,14 +83,14 @@ __global__ __launch_bounds__(256) void gemm_kernel(Args g) {
 		wait_counters<(NS - 2) * (LA + LB + 1), 0>();  // this wave's part of slice kt has landed, its reads of slice kt - 1 are done
 		__syncthreads();
 		fetch(kt + NS - 1, stage == 0 ? NS - 1 : stage - 1);
-		const unsigned char* sl = smem + stage * Rg::STAGE;
-		const unsigned char* sc = sl + Rg::A_BYTES + Rg::B_BYTES;
+		const unsigned char* sl = smem + stage * Ring::STAGE;
+		const unsigned char* sc = sl + Ring::A_BYTES + Ring::B_BYTES;
 		i32x8 fw[RB];
 		int ew[RB];
 #pragma unroll
 		for (int j = 0; j < RB; j++) {
 			const int row = wn * (BN / 2) + w_row(j, l15);
-			const unsigned char* p = sl + Rg::A_BYTES + row * BK;
+			const unsigned char* p = sl + Ring::A_BYTES + row * BK;
 			const i32x4 lo = *reinterpret_cast<const i32x4*>(p + ((q4 ^ swz_w(row)) << 4)), hi = *reinterpret_cast<const i32x4*>(p + (((q4 + 4) ^ swz_w(row)) << 4));
 			fw[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 			ew[j] = sc[256 + row];
@@ -120,13 +120,13 @@ __global__ __launch_bounds__(256) void gemm_kernel(Args g) {
 	wait_vmcnt<0>();  // the loads behind the last slice land in LDS too
 }
 
-template <int BM, int BN, int NS, int FMT>
-static int launch_sized(Args g, hipStream_t stream) {
-	g.tiles_m = (g.M + BM - 1) / BM, g.tiles_n = (g.N + BN - 1) / BN;
+template <int FMT>
+static int launch_64(Args g, hipStream_t stream) {
+	g.tiles_m = (g.M + Ring::BM - 1) / Ring::BM, g.tiles_n = (g.N + Ring::BN - 1) / Ring::BN;
 	const int64_t nwork = (int64_t)g.tiles_m * g.tiles_n * g.splits;
 	ELF_REQUIRE(nwork <= GRID_256, "gemm_fp8: too many tiles for one launch");
-	auto kern = gemm_kernel<BM, BN, NS, FMT>;
-	constexpr int smem = Ring<BM, BN, NS>::BYTES;
+	auto kern = gemm_kernel<FMT>;
+	constexpr int smem = Ring::BYTES;
 	static std::atomic<uint64_t> devices{0};
 	if (int rc = allow_lds(reinterpret_cast<const void*>(kern), smem, devices)) return rc;
 	ELF_LAUNCH(kern, dim3((uint32_t)nwork), dim3(256), smem, stream, g);
@@ -227,7 +227,7 @@ static int launch(const Args& g, const Plan& p, hipStream_t stream) {
 		case FEW: return launch_few<FMT>(g, p.waves, stream);
 		case TILE128: return launch_tile<FMT>(g, 128, stream);
 		case TILE256: return launch_tile<FMT>(g, 256, stream);
-		default: return launch_sized<64, 64, 4, FMT>(g, stream);
+		default: return launch_64<FMT>(g, stream);
 	}
 }
 

@@ -66,31 +66,27 @@ __global__ __launch_bounds__(256, (Tile<RF, CF, NS>::PER_CU)) void gemm_tile_ker
 	}
 	const uint32_t x_lds = lds + T::X_AT + wave * (RF * 1024), w_lds = lds + T::W_AT + ((wave >> 1) * 4 * CF + (wave & 1) * CF) * 1024, s_lds = lds + T::S_AT + wave * 256;
 
-	// What the slices of a tile (of one K range) are loaded from: the operands at its rows (the descriptors' sizes end with the matrix) and the
+	// What the slices of a tile are loaded from: the operands at its rows (the descriptors' sizes end with the matrix) and the
 	// scales of the operand that this wave fetches (even waves: token rows, odd: weight rows; two waves do what one could)
 	struct Source {
 		const uint8_t *x, *w, *s;
 		uint32_t x_bytes, w_bytes, s_bytes;
-		int m0, n0, split, nk;
+		int m0, n0;
 	};
 	const bool s_of_x = (wave & 1) == 0;
 	const int64_t s_step = s_of_x ? g.ldsa : g.ldsb;
-	const int ntiles = g.tiles_m * g.tiles_n, nwork = ntiles * g.splits;
+	const int ntiles = g.tiles_m * g.tiles_n, nk = g.nk;  // nk: at least NS
 	auto source = [&](int pid) {
 		Source t;
-		t.split = pid / ntiles;
 		int tm, tn;
-		tile_at(g, pid - t.split * ntiles, tm, tn);
-		t.split = __builtin_amdgcn_readfirstlane(t.split);
+		tile_at(g, pid, tm, tn);
 		t.m0 = __builtin_amdgcn_readfirstlane(tm * T::M);
 		t.n0 = __builtin_amdgcn_readfirstlane(tn * T::N);
-		const int64_t kt0 = (int64_t)t.split * g.split_nk;
-		t.nk = min(g.split_nk, g.nk - (int)kt0);  // at least NS
-		t.x = g.A + t.m0 * g.lda + kt0 * BK;
-		t.w = g.B + t.n0 * g.ldb + kt0 * BK;
+		t.x = g.A + t.m0 * g.lda;
+		t.w = g.B + t.n0 * g.ldb;
 		t.x_bytes = (uint32_t)((min(T::M, g.M - t.m0) - 1) * g.lda) + BK;
 		t.w_bytes = (uint32_t)((min(T::N, g.N - t.n0) - 1) * g.ldb) + BK;
-		t.s = (s_of_x ? g.sa + t.m0 : g.sb + t.n0) + kt0 * s_step;
+		t.s = s_of_x ? g.sa + t.m0 : g.sb + t.n0;
 		t.s_bytes = scale_bytes(s_of_x ? g.M - t.m0 : g.N - t.n0);
 		return t;
 	};
@@ -98,9 +94,9 @@ __global__ __launch_bounds__(256, (Tile<RF, CF, NS>::PER_CU)) void gemm_tile_ker
 	Source cur = source(pid), nxt = cur;
 
 	// slices nk .. nk + NS - 1 are the next tile's first ones or, behind the workgroup's last tile, its own, which nobody reads
-	auto x_buf = [&](int step) { return step < cur.nk ? buffer_of(cur.x + (int64_t)step * BK, cur.x_bytes) : buffer_of(nxt.x + (int64_t)(step - cur.nk) * BK, nxt.x_bytes); };
-	auto w_buf = [&](int step) { return step < cur.nk ? buffer_of(cur.w + (int64_t)step * BK, cur.w_bytes) : buffer_of(nxt.w + (int64_t)(step - cur.nk) * BK, nxt.w_bytes); };
-	auto s_buf = [&](int step) { return step < cur.nk ? buffer_of(cur.s + step * s_step, cur.s_bytes) : buffer_of(nxt.s + (step - cur.nk) * s_step, nxt.s_bytes); };
+	auto x_buf = [&](int step) { return step < nk ? buffer_of(cur.x + (int64_t)step * BK, cur.x_bytes) : buffer_of(nxt.x + (int64_t)(step - nk) * BK, nxt.x_bytes); };
+	auto w_buf = [&](int step) { return step < nk ? buffer_of(cur.w + (int64_t)step * BK, cur.w_bytes) : buffer_of(nxt.w + (int64_t)(step - nk) * BK, nxt.w_bytes); };
+	auto s_buf = [&](int step) { return step < nk ? buffer_of(cur.s + step * s_step, cur.s_bytes) : buffer_of(nxt.s + (step - nk) * s_step, nxt.s_bytes); };
 
 	int stage = 0, s_stage = 0;  // of the slice that is multiplied; the loads go into stage `stage` and, of scales, into the one before s_stage
 	auto before = [](int s) { return s == 0 ? NS : s - 1; };
@@ -208,24 +204,23 @@ __global__ __launch_bounds__(256, (Tile<RF, CF, NS>::PER_CU)) void gemm_tile_ker
 
 	for (;;) {
 		const int pid_n = pid + (int)gridDim.x;
-		const bool more = pid_n < nwork;
+		const bool more = pid_n < ntiles;
 		if (more) nxt = source(pid_n);
 		slice(std::true_type{}, 0);
-		for (int kt = 1; kt < cur.nk; kt++) slice(std::false_type{}, kt);
+		for (int kt = 1; kt < nk; kt++) slice(std::false_type{}, kt);
 
 		// (the compiler knows nothing of the MFMAs' latency: the last one's result is there after 32 wait states, it needs fewer)
 		asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
 		const int64_t row0 = cur.m0 + wm * 16 * RF + l15;
 		const int col0 = cur.n0 + wn * 32 * CF + 8 * q4;
 		const bool whole = cur.n0 + T::N <= g.N;
-		void* const C = reinterpret_cast<float*>(g.C) + (g.splits > 1 ? (int64_t)cur.split * g.M * g.N : 0);
 #pragma unroll
 		for (int i = 0; i < RF; i++) {
 			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
 			for (int j = 0; j < 2 * CF; j++) asm volatile("" : "+a"(acc[i][j]));  // (a row slab's accumulators are not read before its turn)
-			if (whole) store_row<true, CF>(g, C, row0 + i * 16, col0, acc[i]);
-			else store_row<false, CF>(g, C, row0 + i * 16, col0, acc[i]);
+			if (whole) store_row<true, CF>(g, g.C, row0 + i * 16, col0, acc[i]);
+			else store_row<false, CF>(g, g.C, row0 + i * 16, col0, acc[i]);
 		}
 		if (!more) break;
 		pid = pid_n, cur = nxt;
@@ -238,15 +233,15 @@ template <int RF, int CF, int NS, int FMT>
 static int launch_sized(Args g, hipStream_t stream) {
 	using T = Tile<RF, CF, NS>;
 	g.tiles_m = (g.M + T::M - 1) / T::M, g.tiles_n = (g.N + T::N - 1) / T::N;
-	// (the loads run NS slices ahead, into the next tile's: a K range that had fewer would be read past its end)
-	ELF_REQUIRE(g.split_nk >= NS && g.nk - (int64_t)(g.splits - 1) * g.split_nk >= NS, "gemm_fp8: these tiles need %d blocks of K in every range", NS);
-	const int64_t nwork = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-	ELF_REQUIRE(nwork < (int64_t(1) << 30), "gemm_fp8: too many tiles for one launch");  // (their numbers are ints)
+	// (the loads run NS slices ahead, into the next tile's: a K that had fewer would be read past its end)
+	ELF_REQUIRE(g.nk >= NS && g.splits == 1, "gemm_fp8: these tiles need %d blocks of K in one range", NS);
+	const int64_t ntiles = (int64_t)g.tiles_m * g.tiles_n;
+	ELF_REQUIRE(ntiles < (int64_t(1) << 30), "gemm_fp8: too many tiles for one launch");  // (their numbers are ints)
 	auto kern = gemm_tile_kernel<RF, CF, NS, FMT>;
 	static std::atomic<uint64_t> devices{0};
 	if (int rc = allow_lds(reinterpret_cast<const void*>(kern), T::BYTES, devices)) return rc;
 	constexpr int64_t MOST = 256 * T::PER_CU;
-	ELF_LAUNCH(kern, dim3((uint32_t)(nwork < MOST ? nwork : MOST)), dim3(256), T::BYTES, stream, g);
+	ELF_LAUNCH(kern, dim3((uint32_t)(ntiles < MOST ? ntiles : MOST)), dim3(256), T::BYTES, stream, g);
 	ELF_CHECK_HIP(hipGetLastError());
 	return 0;
 }
@@ -255,8 +250,8 @@ template <int FMT>
 int launch_tile(const Args& g, int tile, hipStream_t stream) {
 	return tile == 256 ? launch_sized<8, 4, 2, FMT>(g, stream) : launch_sized<4, 2, 2, FMT>(g, stream);
 }
-template int launch_tile<FP8_E4M3>(const Args& g, int way, hipStream_t stream);
-template int launch_tile<FP8_E5M2>(const Args& g, int way, hipStream_t stream);
+template int launch_tile<FP8_E4M3>(const Args& g, int tile, hipStream_t stream);
+template int launch_tile<FP8_E5M2>(const Args& g, int tile, hipStream_t stream);
 
 }  // namespace fp8
 }  // namespace elf
