@@ -352,7 +352,9 @@ class Engine:
 		(copies to pinned memory on side streams stay eager), and between replays nothing else may
 		run stage ops of these blocks.  ``warmup`` eager steps run first so that every pool and
 		workspace has its final size (nothing may allocate device memory while capturing); the
-		gradient accumulators are put back as they were, so the capture itself adds no gradient.
+		gradient accumulators are put back as they were, so the capture itself adds no gradient.  A generic stage's
+		``.grad`` tensors are the graph's own from then on, written anew by each replay: autograd adding to one that
+		lay elsewhere would go on writing to that memory after ``zero_grad`` has given it up.
 		"""
 		for op in schedule:
 			if op.op == OperationType.PREFETCH_ACTIVATIONS or op.options.get(OpOptions.ACTIVATION_OFFLOAD):
@@ -360,6 +362,8 @@ class Engine:
 		static_batch = None if batch is None else [t.clone() for t in batch]
 		static_target = None if target is None else target.clone()
 		kept = [[g.clone() for g in getattr(b, "_fused_g", [])] for b in self.blocks]
+		generic = [p for b in self.blocks if not hasattr(b, "_fused_g") for p in b.model.parameters()]
+		kept_main = [p.main_grad.clone() if getattr(p, "main_grad", None) is not None else None for p in generic]
 		side = torch.cuda.Stream()
 		side.wait_stream(torch.cuda.current_stream())
 		with torch.cuda.stream(side):
@@ -371,11 +375,15 @@ class Engine:
 		for b, gs in zip(self.blocks, kept):
 			for g, keep in zip(getattr(b, "_fused_g", []), gs):
 				g.copy_(keep)
+		for p, keep in zip(generic, kept_main):
+			p.grad = None
+			if getattr(p, "main_grad", None) is not None:
+				p.main_grad.zero_() if keep is None else p.main_grad.copy_(keep)
 		graph = torch.cuda.CUDAGraph()
 		with torch.cuda.graph(graph):
 			result, losses, _, _ = self.train_step(static_batch, static_target, loss_fn, schedule, mb_sizes)
 		self._reset_slots()
-		return GraphedStep(graph, static_batch, static_target, result, losses)
+		return GraphedStep(graph, static_batch, static_target, result, losses, [(p, p.grad) for p in generic if p.grad is not None])
 
 	def _reset_slots(self):
 		"""Empty the per-micro-batch slot lists of every block (what Pipeline.step does after a step)."""
@@ -392,10 +400,10 @@ class GraphedStep:
 	"""A captured ``Engine.train_step``.  ``replay(batch, target)`` copies the new data into the
 	buffers the graph reads, launches the graph and returns ``(result, losses)``: the same GPU tensors
 	every time (an eager step moves its outputs to the host), overwritten by each replay.  Weight gradients accumulate into the blocks' ``main_grad``
-	buffers exactly as in an eager step (zero them between steps as usual)."""
+	buffers exactly as in an eager step (zero them between steps as usual); ``grads``: the ``.grad`` tensors that generic stages leave."""
 
-	def __init__(self, graph, batch, target, result, losses):
-		self.graph, self.batch, self.target, self.result, self.losses = graph, batch, target, result, losses
+	def __init__(self, graph, batch, target, result, losses, grads=()):
+		self.graph, self.batch, self.target, self.result, self.losses, self.grads = graph, batch, target, result, losses, grads
 
 	def replay(self, batch=None, target=None):
 		if batch is not None:
@@ -404,6 +412,8 @@ class GraphedStep:
 		if target is not None:
 			self.target.copy_(target)
 		self.graph.replay()
+		for p, grad in self.grads:
+			p.grad = grad
 		return self.result, self.losses
 
 

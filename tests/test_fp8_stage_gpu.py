@@ -355,3 +355,54 @@ def test_norm_over_its_inputs(T, d, over):
 	got = K.rms_norm_fp8(x, gamma, residual=r, h=x if over == "x" else r)
 	assert got[0] is (x if over == "x" else r) and torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
 	assert torch.equal(got[1].q.view(torch.uint8), want[1].q.view(torch.uint8)) and torch.equal(got[1].scale.view(torch.uint8), want[1].scale.view(torch.uint8))
+
+
+# ------------------------------------------------------------------------------------------------ captured
+class _Mixed(nn.Module):
+	def __init__(self, d=128):
+		from elf_amd.models import Linear8, NormLinear8, RMSNorm
+
+		super().__init__()
+		self.norm, self.inner, self.down, self.plain = RMSNorm(d), NormLinear8(d, 200), Linear8(200, d), nn.Linear(d, d)
+
+	def forward(self, x):
+		h, y = self.inner(self.norm(x), x)
+		return h + self.plain(self.down(F.gelu(y)))
+
+
+@pytest.mark.parametrize("scheduler,placement", [("afab", [0, 0]), ("afab", [0])])
+def test_captured_step_of_generic_stages(scheduler, placement):
+	"""Replays give what eager steps give, for the parameters of every kind of layer, with eager steps, ``zero_grad`` and other
+	allocations in between."""
+	from elf_amd.pipeline import Pipeline
+
+	torch.manual_seed(60)
+	stages = [_Mixed().to(torch.bfloat16) for _ in placement]
+	g, mb, n_mb = gen(61), 64, 4
+	draw = lambda: (rnd(g, mb * n_mb, 128), rnd(g, mb * n_mb, 128))
+
+	def loss_fn(pred, target, reduction="sum"):
+		return F.mse_loss(pred.float(), target.float(), reduction=reduction)
+
+	x, tgt = draw()
+	pipe = Pipeline(stages, x[:mb], scheduler=scheduler, partitioner=False, placement=placement)
+	pipe.zero_grad()
+	replay = pipe.capture_step(x, tgt, loss_fn, split_size=mb)
+	for rep in range(4):
+		x, tgt = draw()
+		pipe.zero_grad()
+		others = [torch.full((n,), 7.0, dtype=torch.bfloat16, device="cuda") for n in (128, 200, 72, 128 * 128)]  # (where given-up gradients lay)
+		out, loss = replay(x, tgt)
+		torch.cuda.synchronize()
+		got = [t.clone() for t in out] + [p.grad.clone() for p in pipe.parameters()]
+		got_main = [None if getattr(p, "main_grad", None) is None else p.main_grad.clone() for p in pipe.parameters()]
+		assert all((t == 7).all() for t in others)
+		pipe.zero_grad()
+		want_out, want_loss = pipe(x, tgt, loss_fn, split_size=mb)
+		assert float(loss) == pytest.approx(float(want_loss), rel=1e-4)
+		want = [t.cuda() for t in want_out] + [p.grad for p in pipe.parameters()]
+		names = [f"out {i}" for i in range(len(out))] + [n for n, _ in pipe.named_parameters()]
+		for a, b, name in zip(got, want, names):
+			assert torch.equal(a, b), f"replay {rep}: {name}"
+		for a, p in zip(got_main, pipe.parameters()):
+			assert a is None or torch.equal(a, p.main_grad), f"replay {rep}"
