@@ -7,7 +7,9 @@
 //    vector instruction (with fp32 scales every accumulator would be added to by the vector ALU once per block);
 //  * a value's position between the numbers of the type does not depend on the scale: rows quantized along their columns and along their
 //    rows hold the same values, but for those below 2^-13 (e4m3; e5m2: 2^-28) of their block's largest, which lose bits or vanish;
-//  * the values a block stands for are bf16 numbers (2^128, to which magnitudes from 1.9375 2^127 on round, aside): restoring them rounds nothing.
+//  * the values a block stands for are bf16 numbers where its scale is 2^-117 or more, or where it was made from bf16 (2^128, to which magnitudes
+//    from 1.9375 2^127 on round, aside): restoring them rounds nothing.  The norm's output goes into 8 bits from fp32; e4m3's smallest number
+//    at the smallest scale, 2^-135, lies below bf16's, 2^-133.
 // Scales of the rows of a block lie side by side because a tile of a product reads them for many rows and one block at a time.
 #pragma once
 #include "common.h"

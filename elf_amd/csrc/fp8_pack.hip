@@ -158,7 +158,8 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs g) {
 	}
 }
 
-// Out of 8 bits: 16 lanes a row of a square, 8 values each, so that a row leaves as 256 contiguous bytes.
+// Out of 8 bits: 16 lanes a row of a square, 8 values each, so that a row leaves as 256 contiguous bytes.  The factor rounds nothing (fp32 has
+// 2^-127 times either type's smallest number, 2^-143); bf16 rounds what its subnormal numbers do not hold, where a scale is below 2^-117.
 template <int FMT>
 __global__ __launch_bounds__(256) void dequant_kernel(PackArgs g, bf16_t* out, int64_t ldo) {
 	const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(256) void dequant_kernel(PackArgs g, bf16_t* out, i
 		const float scale = fp8_scale(byte[p]);
 		bf16x8 o;
 #pragma unroll
-		for (int j = 0; j < 8; j++) o[j] = (bf16_t)(u[j >> 2][j & 3] * scale);  // exact (2^128 becomes an infinity)
+		for (int j = 0; j < 8; j++) o[j] = (bf16_t)(u[j >> 2][j & 3] * scale);  // (2^128 becomes an infinity)
 		const u32x4 v = __builtin_bit_cast(u32x4, o);
 		uint32_t next = 0;
 		if (g.between) next = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[0], 0x101, 0xf, 0xf, false);  // row_shl 1: the lane behind

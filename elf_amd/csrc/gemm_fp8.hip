@@ -8,8 +8,8 @@ namespace fp8 {
 constexpr int64_t MOST = (int64_t(1) << 31) - 512;  // M, N and K
 
 // 64 x 64 tiles: four waves, 2 x 2, each 32 x 32; a ring of four K slices in LDS, filled by direct-to-LDS loads three slices ahead.
-// Bound: the chain barrier -> fragment reads -> MFMAs of a slice, 0.32 us and 0.45 for two workgroups of a compute unit (four
-// slices in LDS; two slices 0.53 and 0.54, eight 0.38).
+// Bound: alone on a compute unit by the chain barrier -> fragment reads -> MFMAs of a slice, 0.32 us (two slices in LDS 0.53, eight 0.38); two workgroups
+// take 0.45, 73 KB/us into LDS (two slices 0.54).
 // A slice of an operand is its rows' 128 bytes of one block, 16-byte chunk c of row r in place c ^ f(r) so that the 16 lanes of a
 // fragment read meet 16 different bank groups, and one scale byte a row.  Rows behind the matrix are zeros.
 // A lane's share of a fragment is the chunks q and q + 4 of its row, q = lane / 16: the order of k within a block is free, as long as both
@@ -172,7 +172,9 @@ __global__ __launch_bounds__(256) void join_kernel(Args g, const float* __restri
 //   64 x 64 / 128 x 128 / 256 x 256: 79 x 26244 x 228 8.0 / 6.8 / 10.4, 5827 x 2080 x 162 19.5 / 12.5 / 12.6, 256 x 4096 x 4096 12.5 / 17.3 / 40,
 //     512 x 4096 x 4096 16.1 / 17.5 / 40.7, 1024 x 4096 x 4096 29 / 19.3 / 41, 2111 x 4288 x 1600 32 / 21.0 / 24.9, 1625 x 14312 x 3520 157 / 96 / 85,
 //     2048 x 6144 x 4096 99 / 53 / 44.8, 4096 x 6144 x 4096 189 / 106 / 92, 8192 x 28672 x 4096 1678 / 955 / 689
-// Over 638 drawn sizes of 1 to 8192 rows, 64 to 28672 columns and K up to 14336 the way taken is 1.1 % slower than the fastest (geometric mean; 20 % at most).
+// Over 638 drawn sizes of 1 to 8192 rows, 64 to 28672 columns and K up to 14336 the way taken was 1.1 % slower than the fastest (geometric mean; 20 % at most), in a build
+// of its own that could be told the way.  All of it is of bf16 outputs without a residual, and so is the memory that `out` counts: a
+// residual or fp32 outputs move twice as much, fp32 sums four times.
 // (128 x 256 tiles lay within 5 % of the better of their neighbours, 64 x 128 within 10 %; K ranges of 128 x 128 and 256 x 256 tiles never paid.)
 struct Plan {
 	int way, waves, splits, split_nk;

@@ -16,7 +16,9 @@ namespace fp8 {
 // Measured: 8192 x 28672 x 4096 on 256 x 256 tiles 669 to 730 us from part to part, 2.9 to 2.6 PFLOP/s (8192^3 2.9; the vendor's product of
 // matrices with one scale each 2.75): bound by power, the matrix pipe busy 71 % of the cycles at 1.57 GHz, no LDS bank conflict.  64 tiles alone
 // take 1.25 us a slice at full clock, 0.97 with operands in L2, for 0.85 of MFMAs.  128 x 128 tiles: 0.6 us a slice, 1.0 for two workgroups of a
-// compute unit, bound by the trip of a load (0.26 us of MFMAs a slice).  Not faster, at the same 128 x 128 and on 128 x 256: three and four slices in LDS, one
+// compute unit (0.26 us of MFMAs a slice each): bound by the rate at which a compute unit is served, 50 to 73 KB/us on tiles of every size, for more
+// slices in LDS gain nothing.  2111 x 4287 x 1599, 26 us: matrix pipe busy 29 % of the cycles, the path of returning loads 67 % (half of that it waits), L1 waits for
+// L2 30 %, L2 hits 82 %.  Not faster, at the same 128 x 128 and on 128 x 256: three and four slices in LDS, one
 // barrier a slice with both operands' fragments a slice ahead, eight waves; on 256 x 256: barriers earlier and later, weight fragments read earlier.
 template <int RF, int CF, int NS>
 struct Tile {
