@@ -215,9 +215,9 @@ class _Use:
 
 class _Kept8:
 	"""What a layer in 8 bits keeps of a micro-batch: its input or its output gradient along the tokens (``kernels.Fp8Rows`` of the
-	transpose, half of the bf16 bytes), and of an output gradient its sum over the tokens where there is a bias and the gradient of the gain where
-	there is a norm, both in fp32.  ``use``: the forward call it belongs to; ``more``: what came before it of the same call (a
-	stage goes back from its outputs one after the other)."""
+	transpose: half of the bf16 bytes, with the tokens filled up to 128), and of an output gradient its sum over the tokens where there is a
+	bias and the gradient of the gain where there is a norm, both in fp32.  ``use``: the forward call it belongs to; ``more``: what came
+	before it of the same call (a stage goes back from its outputs one after the other)."""
 
 	__slots__ = ("rows", "bias", "gain", "use", "more")
 
