@@ -205,7 +205,7 @@ int elf_dequant_fp8(const void* q, int64_t ldq, const void* s, int64_t lds, int6
 /* RMSNorm with the residual's addition in front and 8 bits behind it: h[T, d] = x + residual (bf16, rounded once; residual NULL: x is
  * normalized and h is not written), y = h * rsqrt(mean(h^2) + eps) * gamma in fp32, and y along its rows in 8 bits (q, s).  stats
  * [T, 2] = {0, 1 / rms}: the backward is elf_norm_bwd over h, whose dres is h's own gradient and whose dx is that of x and of the
- * residual alike.  d a multiple of 8, at most 8192; dense rows, 16-byte aligned; h may be x or the residual. */
+ * residual alike.  d a multiple of 8, at most 8192; dense rows, 16-byte aligned; h may be x or the residual, but overlaps neither otherwise. */
 int elf_rms_norm_fp8(const void* x, const void* residual, const void* gamma, void* h, void* q, int64_t ldq, void* s, int64_t lds,
                      void* stats, int64_t T, int d, float eps, int fmt, void* stream);
 /* C[M, N] (+)= A B^T for A[M, K] and B[N, K] in 8 bits, with fp32 sums: A of either type, B e4m3.  (The matrix instruction adds the

@@ -339,6 +339,10 @@ def test_norm_into_given_memory():
 		assert got[0] is h and torch.equal(h, want[0]) and all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip((got[1].q, got[1].scale), (want[1].q, want[1].scale))) and torch.equal(got[2], want[2])
 	with pytest.raises(ElfStageError, match="h must be dense"):
 		K.rms_norm_fp8(x, gamma, residual=r, h=torch.empty(20, 80, dtype=torch.bfloat16, device="cuda")[:, :72])
+	both = rnd(g, 21, 72)
+	for x2, r2, h2 in ((both[:20], r, both[1:]), (x, both[1:], both[:20])):
+		with pytest.raises(ElfStageError, match="shifted"):
+			K.rms_norm_fp8(x2, gamma, residual=r2, h=h2)
 	with pytest.raises(ElfStageError, match="x itself"):
 		K.rms_norm_fp8(x, gamma, h=torch.empty_like(x))
 
