@@ -327,8 +327,9 @@ class Linear8DW(LayerDW, Linear8):
 
 
 class NormLinear8DX(torch.autograd.Function):
-	"""(h, y) of ``NormLinear8`` (y alone without a residual).  B reads h again: where h was written in place, autograd refuses.  It hands the norm's backward the product's result, in bf16 as every layer's input
-	gradient, and h's own gradient.  The gain's gradient of a micro-batch goes through autograd, rounded, and is kept in fp32 for W."""
+	"""(h, y) of ``NormLinear8`` (y alone without a residual).  B reads h again: where h was written in place, autograd refuses.  It hands the
+	norm's backward the product's result, in bf16 as every layer's input gradient, and h's own gradient.  The gain's gradient of a
+	micro-batch goes through autograd, rounded, and is kept in fp32 for W."""
 
 	@staticmethod
 	def forward(ctx, x, residual, gamma, weight, bias, linear):
