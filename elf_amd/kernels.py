@@ -540,7 +540,7 @@ def rms_norm_fp8(x, gamma, residual=None, eps=1e-5, dtype=torch.float8_e4m3fn, h
 			h = torch.empty(shape, dtype=torch.bfloat16, device=device)
 		elif h.shape != shape or h.dtype != torch.bfloat16 or not h.is_contiguous() or h.get_device() != index:
 			raise _lib.ElfStageError(f"rms_norm_fp8: h must be dense and of x's shape {tuple(shape)} in bfloat16 on {device}, got {h.dtype} {tuple(h.shape)} on {h.device}")
-		elif any(0 < abs(h.data_ptr() - t) < 2 * T * d for t in (x.data_ptr(), r)):
+		elif 0 < abs(h.data_ptr() - x.data_ptr()) < 2 * T * d or 0 < abs(h.data_ptr() - r) < 2 * T * d:
 			raise _lib.ElfStageError("rms_norm_fp8: h may be x's or the residual's memory, not a part of it shifted against theirs")
 	y = Fp8Rows.empty(T, d, dtype, device)
 	stats = torch.empty((T, 2), dtype=torch.float32, device=device)
